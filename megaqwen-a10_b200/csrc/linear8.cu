@@ -396,6 +396,7 @@ __device__ __forceinline__ void epilogue_channels(const GemmParams& P, uint32_t 
 #pragma unroll 1
     for (int j = 0; j < BN && t0 + j < P.M; j += 16) {
         int v[16];
+        __syncwarp();            // the lanes without a channel skipped the stores
         tmem_ld16(at + j, v);
         const int n = min(16, P.M - t0 - j);
         if (ch < P.N) {
@@ -637,8 +638,10 @@ __global__ void __launch_bounds__(Gemm<BN>::THREADS, 1) gemm_kernel(const __grid
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            __syncwarp();        // before the next tile's barrier
         }
     }
+    __syncwarp();                // one lane ran the roles of warps 0 and 1: the aligned barriers below take whole warps
     if (S > 1) {
         // every CTA of the cluster adds up its share of the tokens
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -666,6 +669,7 @@ __global__ void __launch_bounds__(Gemm<BN>::THREADS, 1) gemm_kernel(const __grid
                         store_elem(P.out, (long long)(t0 + j) * P.N + n0 + c4 + k, P.out_dtype, (float)v[k] * (sx * P.ws[n0 + c4 + k]));
             }
         }
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     tc_fence_before();
