@@ -415,6 +415,7 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
             }
 
             ok = wait(&s_done, ns++) && ok;
+            __syncwarp();                              // the waits of a warp's lanes end one by one; the loads take the whole warp
             tc_fence_after();
             float s[32];
             tmem_ld32(tmem + lanes + 32 * half, s);
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
 #pragma unroll 1
         for (int e = 0; e < D / 64; ++e) {         // blocks of 32 dims
             float o[32];                           // [j][r]
+            __syncwarp();                          // rows that do not exist skipped the stores
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float x[8];
