@@ -478,24 +478,25 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                 }
         };
 
-        for (int u = cur.u; u < cur.u1; ++u) {
+        for (int u = cur.u; u < cur.u1 && !dead; ++u) {
             const int p0 = u * TP, st = nuse % NST;
-            if (!dead) {
-                bool late = false;
-                if (!mbar_test(&bars[warp][st], (nuse / NST) & 1)) {
-                    const unsigned long long t0 = globaltimer();
-                    while (!mbar_test(&bars[warp][st], (nuse / NST) & 1))
-                        if (globaltimer() - t0 > WAIT_NS) { late = true; break; }
-                }
-                dead = __any_sync(0xffffffffu, late);
-                if (dead && lane == 0) report(P.c, MQ_DEV_TIMEOUT_RING, blockIdx.x);
+            bool late = false;
+            if (!mbar_test(&bars[warp][st], (nuse / NST) & 1)) {
+                const unsigned long long t0 = globaltimer();
+                while (!mbar_test(&bars[warp][st], (nuse / NST) & 1))
+                    if (globaltimer() - t0 > WAIT_NS) { late = true; break; }
+            }
+            dead = __any_sync(0xffffffffu, late);
+            if (dead) {              // this tile and those after it are not counted as used: the end waits for their copies
+                if (lane == 0) report(P.c, MQ_DEV_TIMEOUT_RING, blockIdx.x);
+                break;
             }
             const uint8_t* base = ring + st * G::STAGE;
             if (p0 + TP <= low) tile(std::false_type{}, base, p0);
             else if (p0 < high) tile(std::true_type{}, base, p0);
             ++nuse;
             __syncwarp();        // every lane has read the stage before it is filled again
-            if (!dead && u + NST < cur.u1) load(b, h, len, u + NST);
+            if (u + NST < cur.u1) load(b, h, len, u + NST);
         }
         // the next segment's copies and queries are under way while this one's warps meet
         const Segment seg = cur;
