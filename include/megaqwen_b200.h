@@ -414,8 +414,8 @@ int mq_kv4_read(const MQKV4Cache* cache, const int* starts, int n, int dtype, vo
  *     at position lengths[b] - counts[b] + t and sees positions 0 .. its own; a
  *     row with t >= counts[b], or before position 0, gives zeros.
  *   - workspace (scratch) and counters (int32, zero before the first use, left
- *     zero): as large as mq_kv4_attend_workspace says; calls that may overlap
- *     need their own.
+ *     zero): as large as mq_kv4_attend_workspace says; calls on different
+ *     streams need their own, host threads on one stream may share them.
  *   - batch <= 4096.
  */
 int mq_kv4_attend_workspace(const MQKV4Cache* cache, int tokens, int num_q_heads, size_t* bytes, size_t* counters);
@@ -432,8 +432,8 @@ int mq_kv4_attend(const MQKV4Cache* cache, int dtype, const void* q, const int64
  *     rounded up to 16, whose bytes up to there are readable (their values do not
  *     matter), 16-byte aligned; w_scale: fp32 [N]; out: [M][N] of out_dtype,
  *     contiguous; K <= 131072.
- *   - workspace: mq_linear8_workspace_bytes(M, K) bytes, 16-byte aligned; calls that
- *     may overlap need their own.
+ *   - workspace: mq_linear8_workspace_bytes(M, K) bytes, 16-byte aligned; calls on
+ *     different streams need their own, host threads on one stream may share it.
  *   - status: device int32 [2], zero before the first use: an MQ_DEV_* code if a
  *     bounded wait ran out.
  */

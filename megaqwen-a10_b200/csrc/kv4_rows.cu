@@ -19,6 +19,7 @@
 // scores into weights (49 % of the issue slots with two CTAs on an SM) between barriers; the queries 4 us at the start,
 // the joins 5 at the end.
 #include "kv4_plan.cuh"
+#include "launch_lock.h"
 
 namespace mq {
 namespace kv4 {
@@ -630,6 +631,7 @@ int launch(const RowsParams& p, unsigned grid, cudaStream_t stream) {
             return (int)e;
         set[dev] = true;
     }
+    const LaunchLock lock(p.a.part);   // the join reads what this call's first kernel left
     const int rc = launch_pdl(rows_kernel<D, GS>, grid, NTHR, fixed + ((size_t)p.a.c.batch + 1) * 4, stream, p);
     if (rc != MQ_OK) return rc;
     const unsigned items = (unsigned)p.a.c.batch * p.a.c.heads * p.a.blocks;

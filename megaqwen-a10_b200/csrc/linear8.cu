@@ -24,6 +24,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "launch_lock.h"
 
 namespace mq {
 namespace lin8 {
@@ -1095,6 +1096,7 @@ extern "C" int mq_linear8(const void* x, int dtype, int64_t x_stride, const int8
     const size_t codes = round_up((size_t)M * ldq, 256);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < codes + (size_t)M * 4) return MQ_ERR_SIZE;
     QuantParams q{x, x_stride, dtype, vec, M, K, ldq, (int8_t*)workspace, (float*)((uint8_t*)workspace + codes)};
+    const LaunchLock lock(workspace);   // the product reads the codes of this call's quantiser
     if ((rc = launch_quantize(q, stream)) != MQ_OK) return rc;
     GemmParams p{q.scale, w_scale, out, status, out_dtype, M, N, K, 0, 0, 1, 0, 128};
     // Pairs of CTAs where there is a tile for every pair.

@@ -18,6 +18,7 @@ by `check_device`, as the decoders report theirs.  A quantisation group that hol
 an infinity or a NaN reads back as NaN.
 """
 import ctypes
+import threading
 
 import torch
 
@@ -97,7 +98,7 @@ class KV4Cache:
                            head_dim, group)
             self._views.append(v)
             self._refs.append(ctypes.byref(v))
-        self._sizes, self._spaces = {}, {}
+        self._sizes, self._spaces, self._lock = {}, {}, threading.Lock()
         self._seq_shape, self._index, self._scale = torch.Size((batch,)), self.device.index, head_dim ** -0.5
 
     # -- arguments ---------------------------------------------------------
@@ -197,20 +198,20 @@ class KV4Cache:
         args = self._sizes.get((key, tokens, heads))
         if args is None or graph:
             nbytes, ncnt = ctypes.c_size_t(0), ctypes.c_size_t(0)
-            with torch.cuda.device(self.device):
+            with self._lock, torch.cuda.device(self.device):
                 _lib.check(self._lib.mq_kv4_attend_workspace(ref, tokens, heads, ctypes.byref(nbytes), ctypes.byref(ncnt)),
                            "mq_kv4_attend_workspace")
-            have = None if graph else self._spaces.get(key)
-            if have is None or have[0].numel() < nbytes.value or have[1].numel() < ncnt.value:
-                have = (torch.empty(nbytes.value, dtype=torch.uint8, device=self.device),
-                        torch.zeros(ncnt.value, dtype=torch.int32, device=self.device))
+                have = None if graph else self._spaces.get(key)
+                if have is None or have[0].numel() < nbytes.value or have[1].numel() < ncnt.value:
+                    have = (torch.empty(nbytes.value, dtype=torch.uint8, device=self.device),
+                            torch.zeros(ncnt.value, dtype=torch.int32, device=self.device))
+                    if not graph:
+                        self._spaces[key] = have
+                        for other in [k for k in list(self._sizes) if k[0] == key]:   # they hold the old one's address
+                            del self._sizes[other]
+                args = (have[0].data_ptr(), have[0].numel(), have[1].data_ptr(), have[1].numel()), have
                 if not graph:
-                    self._spaces[key] = have
-                    for other in [k for k in self._sizes if k[0] == key]:   # they hold the old one's address
-                        del self._sizes[other]
-            args = (have[0].data_ptr(), have[0].numel(), have[1].data_ptr(), have[1].numel()), have
-            if not graph:
-                self._sizes[key, tokens, heads] = args
+                    self._sizes[key, tokens, heads] = args
         return args
 
     def status(self):
