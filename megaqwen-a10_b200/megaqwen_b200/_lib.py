@@ -19,6 +19,7 @@ MQ_ERRORS = {
     -6: "the kernel reported a device-side error",
 }
 ROW_PAD = 16  # padding bytes after every weight row in the layout the decoder classes use
+MQ_DEV_BAD_TOKEN = 3
 MQ_DEV_ERRORS = {1: "exchange wait timed out", 2: "weight-ring wait timed out", 3: "invalid token",
                  4: "invalid position", 5: "activation outside the fp16 operand range",
                  6: "page table entry outside the cache"}

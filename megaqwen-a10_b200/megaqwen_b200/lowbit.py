@@ -9,6 +9,7 @@ Norms, the rotation and SiLU are torch operations in fp32; the residual stream i
 """
 import torch
 
+from . import _lib
 from .config import HEAD_DIM, HIDDEN_SIZE, INTERMEDIATE_SIZE, KV_SIZE, NUM_KV_HEADS, NUM_Q_HEADS, Q_SIZE, RMS_EPS, VOCAB_SIZE
 from .kv4 import KV4Cache
 from .linear8 import Int8Linear
@@ -46,6 +47,7 @@ class LowBitDecoder:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self._host_lengths = [0] * batch
+        self.status_ = torch.zeros(2, dtype=torch.int32, device=self.device)   # MQ_DEV_BAD_TOKEN and the sequence
 
     def reset(self):
         self.lengths.zero_()
@@ -101,14 +103,30 @@ class LowBitDecoder:
         self.tokens = logits.argmax(-1).int()
         return logits
 
+    def _ids(self, tokens):
+        """int32 [B] on the device from a list or tensor of token ids.  What is on the host is checked here; a bad
+        one on the device becomes token 0 there and is left in the status word, without a synchronisation."""
+        t = torch.as_tensor(tokens)
+        if t.shape != (self.cache.batch,):
+            raise ValueError("one token for each sequence expected")
+        bad = ~((t >= 0) & (t < VOCAB_SIZE))               # before the cast to 32 bits, which could wrap
+        if t.device.type == "cpu":
+            if bad.any():
+                raise ValueError("token out of range")
+            return t.int().to(self.device)
+        if t.device != self.device:
+            raise ValueError(f"tokens: on {t.device}, expected {self.device}")
+        first = bad.int().argmax().int()
+        self.status_.copy_(torch.where(bad.any(), torch.stack([torch.full_like(first, _lib.MQ_DEV_BAD_TOKEN), first]), self.status_))
+        return t.masked_fill(bad, 0).int()
+
     def step(self, tokens=None):
         """Appends one token for each sequence (default: the last greedy choices) and returns fp32 logits [B, vocab];
-        `tokens` holds the new greedy choices.  No host synchronisation."""
+        `tokens` holds the new greedy choices.  No host synchronisation.  A token outside the vocabulary raises; one in a
+        tensor on the device is reported by `check_device`, and its sequence's logits mean nothing."""
         if max(self._host_lengths) >= self.max_seq_len:
             raise ValueError("KV cache full")
-        ids = self.tokens if tokens is None else torch.as_tensor(tokens, dtype=torch.int32).to(self.device)
-        if ids.shape != (self.cache.batch,):
-            raise ValueError("one token for each sequence expected")
+        ids = self.tokens if tokens is None else self._ids(tokens)
         logits = self._logits(self._forward(ids[:, None], None)[:, 0])
         self._host_lengths = [n + 1 for n in self._host_lengths]
         self.tokens = logits.argmax(-1).int()
@@ -126,6 +144,11 @@ class LowBitDecoder:
         return torch.stack(out, 1).tolist()
 
     def check_device(self):
+        """Raises (and clears the status) if a call met a token, position or page that does not exist, or a wait ran out."""
+        code, info = self.status_.tolist()
+        if code:
+            self.status_.zero_()
+            raise _lib.MQError(f"low-bit decoder: device error {code} ({_lib.MQ_DEV_ERRORS.get(code, '?')}, sequence {info})")
         self.cache.check_device()
         for L in self.layers:
             for n in ("qkv", "o", "gu", "down"):
