@@ -141,7 +141,7 @@ class LowBitDecoder:
             self.step()
             out.append(self.tokens)
         self.check_device()
-        return torch.stack(out, 1).tolist()
+        return torch.stack(out, 1)[:, :max(0, max_new_tokens)].tolist()
 
     def check_device(self):
         """Raises (and clears the status) if a call met a token, position or page that does not exist, or a wait ran out."""
