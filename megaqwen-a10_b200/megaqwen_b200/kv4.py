@@ -100,6 +100,7 @@ class KV4Cache:
             self._refs.append(ctypes.byref(v))
         self._sizes, self._spaces, self._lock = {}, {}, threading.Lock()
         self._seq_shape, self._index, self._scale = torch.Size((batch,)), self.device.index, head_dim ** -0.5
+        torch.cuda.current_stream(self.device).synchronize()   # the fills are done, whatever stream the first call is on
 
     # -- arguments ---------------------------------------------------------
     def _layer(self, layer):

@@ -46,6 +46,7 @@ class Int8Linear:
         self._fn = _lib.load().mq_linear8
         self._index = self.device.index
         self._fixed = (weight.data_ptr(), weight.stride(0), self.weight_scale.data_ptr(), self.status_.data_ptr())
+        torch.cuda.current_stream(self.device).synchronize()   # the copies are done, whatever stream the first call is on
 
     def __call__(self, x, out_dtype=None):
         """x [..., K] (bf16, fp16 or fp32, contiguous last axis) -> y [..., N] of out_dtype (default: x's type)."""

@@ -48,6 +48,7 @@ class LowBitDecoder:
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self._host_lengths = [0] * batch
         self.status_ = torch.zeros(2, dtype=torch.int32, device=self.device)   # MQ_DEV_BAD_TOKEN and the sequence
+        torch.cuda.current_stream(self.device).synchronize()
 
     def reset(self):
         self.lengths.zero_()
