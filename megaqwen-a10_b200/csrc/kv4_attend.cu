@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
     // First copies of a segment.
     auto open = [&](const Segment& c) {
         if (dead || c.u >= c.u1) return;
-        const int len = min(max(P.lengths[c.b], 0), P.c.max_seq);
+        const int len = positions_of(P, c.b);
         if (P.c.table) {
             page0 = (c.u * TP) >> P.c.page_shift;
             pages = page0 + lane < P.c.pages_per_seq ? P.c.table[(long long)c.b * P.c.pages_per_seq + page0 + lane] : 0;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
     // pairs (0,4), (1,5) / 16, (2,6), (3,7) / 16), the groups' sums, the factor that undoes it all, the row's limit.
     auto stage_q = [&](const Segment& c) {
         const int row0 = c.rb * RB, nrows = min(RB, P.rows - row0);
-        const int len = min(max(P.lengths[c.b], 0), P.c.max_seq);
+        const int len = positions_of(P, c.b);
         const int count = P.counts ? min(max(P.counts[c.b], 0), P.tokens) : P.tokens;
         constexpr int V = D / 32;     // dims of a lane
 #pragma unroll 1
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
         // ------------------------------------------------------------------ one segment
         const int b = cur.b, h = cur.h;
         const int row0 = cur.rb * RB, nrows = min(RB, P.rows - row0);
-        const int len = min(max(P.lengths[b], 0), P.c.max_seq);
+        const int len = positions_of(P, b);
         float acc[NB][NG][2][4];
         // of this lane's score columns 2c + i (row (2c + i) % CR of block nb, group (2c + i) / CR where the groups have
         // columns of their own): reference, sum of weights, q's factor, -8 sum q of the groups
@@ -492,8 +492,10 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                 break;
             }
             const uint8_t* base = ring + st * G::STAGE;
-            if (p0 + TP <= low) tile(std::false_type{}, base, p0);
-            else if (p0 < high) tile(std::true_type{}, base, p0);
+            if (p0 < high) {         // low: the greatest number where every row is padding
+                if (p0 + TP <= low) tile(std::false_type{}, base, p0);
+                else tile(std::true_type{}, base, p0);
+            }
             ++nuse;
             __syncwarp();        // every lane has read the stage before it is filled again
             if (u + NST < cur.u1) load(b, h, len, u + NST);

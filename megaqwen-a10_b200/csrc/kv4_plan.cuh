@@ -66,6 +66,12 @@ __device__ __forceinline__ void scale4(float4& v, float k) { v.x *= k; v.y *= k;
 __device__ __forceinline__ void add4(float4& v, const float4& a, float k) {
     v.x = fmaf(a.x, k, v.x); v.y = fmaf(a.y, k, v.y); v.z = fmaf(a.z, k, v.z); v.w = fmaf(a.w, k, v.w);
 }
+// Positions of sequence b that its rows can see: none where no row of the call is its token, and then nothing of the
+// sequence is needed, whatever its length says.
+__device__ __forceinline__ int positions_of(const AttendParams& P, int b) {
+    const int len = P.lengths[b], count = P.counts ? P.counts[b] : 1;      // two loads at once
+    return count > 0 ? min(max(len, 0), P.c.max_seq) : 0;
+}
 // Four dims of an output row from the sum of weights L (0: the row saw nothing).
 __device__ __forceinline__ void store_out(const AttendParams& P, int b, int h, int row, int D, int d, float4 o, float L) {
     const int t = row / P.share, j = row - t * P.share;
@@ -146,7 +152,7 @@ __device__ __forceinline__ unsigned scan_costs(const AttendParams& P, unsigned* 
         if (b < P.c.batch) {
             const int len = P.lengths[b];
             if (len < 0 || len > P.c.max_seq) report(P.c, MQ_DEV_BAD_POSITION, b);
-            n = (unsigned)(max(1, (min(max(len, 0), P.c.max_seq) + TP - 1) / TP) + OVER);
+            n = (unsigned)(max(1, (positions_of(P, b) + TP - 1) / TP) + OVER);
         }
         most = max(most, n);
         unsigned x = n;

@@ -207,16 +207,15 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
             bulk_g2s(base + dst + (from - p0) * row_bytes, src + r * row_bytes, (to - from) * row_bytes, bar);
         }
     };
-    auto length = [&](int b) { return min(max(P.lengths[b], 0), P.c.max_seq); };
     auto open = [&](const Segment& c) {
-        const int len = length(c.b);
+        const int len = positions_of(P, c.b);
         for (int i = 0; i < STAGES && c.seg0 + 2 * i < c.seg1; ++i) load(c.b, c.h, len, (c.seg0 + 2 * i) * TP, c.seg1 * TP);
     };
     if (more) open(cur);
 
     while (more && !dead) {
         const Segment seg = cur;
-        const int b = seg.b, h = seg.h, row0 = seg.rb * ROWS, nrows = min(ROWS, P.rows - row0), len = length(b);
+        const int b = seg.b, h = seg.h, row0 = seg.rb * ROWS, nrows = min(ROWS, P.rows - row0), len = positions_of(P, b);
         const int count = P.counts ? min(max(P.counts[b], 0), P.tokens) : P.tokens;
         const int end = min(len, seg.seg1 * TP);         // of this segment's positions
         // ------------------------------------------------------------------ queries: 16 rows to a warp, 8 lanes to a row
