@@ -138,17 +138,18 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
-    if (warp == 0) {
-        const unsigned most = scan_costs(P, s_prefix, lane);
-        if (lane == 0) s_max = most;
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     // Only now that this CTA has its TMEM: a later kernel of the stream that allocates some could otherwise take what a
     // CTA of this one still has to get, and wait for that CTA.
     pdl_launch_dependents();
+    pdl_wait();
+    if (warp == 0) {
+        const unsigned most = scan_costs(P, s_prefix, lane);
+        if (lane == 0) s_max = most;
+    }
+    __syncthreads();
     const uint32_t tmem = s_tmem, lanes = (uint32_t)(32 * (warp & 3)) << 16;
     Plan<1> plan{s_prefix, P.c.heads * P.blocks, P.blocks, 0, 0};
     const int per = plan.per, B = P.c.batch;
