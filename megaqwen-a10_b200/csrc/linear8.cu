@@ -642,8 +642,8 @@ __global__ void __launch_bounds__(Gemm<BN>::THREADS, 1) gemm_kernel(const __grid
             __syncwarp();        // before the next tile's barrier
         }
     }
-    __syncwarp();                // one lane ran the roles of warps 0 and 1: the aligned barriers below take whole warps
     if (S > 1) {
+        __syncwarp();            // one lane ran the roles of warps 0 and 1: the aligned barriers below take whole warps
         // every CTA of the cluster adds up its share of the tokens
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (!s_abort) {
