@@ -8,11 +8,13 @@
 // other's waits.  Items cut between CTAs leave partials, which a second kernel joins (a partial is 128 rows, too much
 // for one CTA to join at the end).
 //
-// Arithmetic.  A value code * scale has 3 + 8 significant bits and is exact in fp16 once its position's largest scale
-// is brought to [1, 2) by a power of two: the operands are those quotients, the powers go to the scores (K) and into
-// the weights' exponents (V).  q is fp16 of q 2^-e as in kv4_attend.cu.  Weights are exp2 in fp32 against a reference
-// per row, rounded to fp16 for the product, summed in fp32 unrounded.  The reference moves (and O is scaled) when a
-// weight exceeds 2^15.
+// Arithmetic.  A value code * scale has 3 + 8 significant bits.  Its operand is that value with the position's largest
+// scale brought to [2^12, 2^13) by a power of two, which keeps 7 times it within fp16: exact for the groups whose scale is
+// at least 2^-29 of the position's largest, rounded to 2^-37 of it below that (V: in single-token attention the product
+// with the weight is rounded to 2^-32 of the row's largest; K: there each group's sum is in fp32).  The powers go to the
+// scores (K) and into the weights' exponents (V).  q is fp16 of q 2^-e as in kv4_attend.cu.  Weights are exp2 in fp32
+// against a reference per row, rounded to fp16 for the product (11 bits down to 2^-21 of the largest), summed in fp32
+// unrounded.  The reference moves (and O is scaled) when a weight exceeds 2^15.
 //
 // Measured: 4 sequences of 1000 to 6001 positions, 64 tokens each, 16 heads over 8 of 128 dims: 39.5 us with the joins
 // (88 TFLOP/s; the products alone would take 2 us).  A tile takes a CTA 3.2 us, most of it turning codes into operands and
@@ -26,6 +28,7 @@ namespace kv4 {
 namespace {
 
 constexpr int ROWS = ROWS_BLOCK, TILE = 64, NTHR = 256, STAGES = 2;
+constexpr int LIFT = 12;             // log2 of what a position's largest scale is brought to: 7 * 2^(LIFT + 1) < 65504
 constexpr unsigned WHOLE_UNITS = 8;  // units up to which one CTA takes a whole item
 constexpr int TMEM_COLS = 256, O_COL = 128;
 
@@ -116,8 +119,8 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
     uint8_t* s_v = s_k + G::K;
     uint8_t* s_p = s_v + G::V;
     uint8_t* raw = s_p + G::PT;
-    float* kf = reinterpret_cast<float*>(raw + STAGES * G::RAW);   // [TILE] 2^e of the position's K scales
-    float* ve = kf + TILE;                                          // [TILE] e of its V scales
+    float* kf = reinterpret_cast<float*>(raw + STAGES * G::RAW);   // [TILE] 2^e: K is 2^e times its operand
+    float* ve = kf + TILE;                                          // [TILE] e: V is 2^e times its operand
     float* vi = ve + TILE;                                          // [TILE] 2^-e
     __half* v16 = reinterpret_cast<__half*>(vi + TILE);             // [NS][TILE] V scales * 2^-e
     float* s_mul = reinterpret_cast<float*>(v16 + NS * TILE);       // [ROWS]
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
                         if (x[i] < 0x7f80u) e = max(e, x[i]);
                         else nan |= 1u << i;
                     }
-                    const int ex = min(max((int)(e >> 7), 67) - 127, 126);
+                    const int ex = min(max((int)(e >> 7), 67) - 127, 126) - LIFT;
                     const float down = __uint_as_float((unsigned)(127 - ex) << 23);
 #pragma unroll
                     for (int i = 0; i < NS; ++i) w[i] = __uint_as_float(x[i] << 16) * down;
