@@ -13,11 +13,11 @@
 // Arithmetic.  Scores: S^T = K q^T by m16n8k16 fp16 products with fp32 sums; 16 positions are the rows of A,
 // 8 query rows the columns (an A with the queries as rows would be half empty for up to 8 of them).  A K code
 // enters as the fp16 subnormal nibble * 2^-24, which a mask alone makes (16 nibble * 2^-24 for every other one,
-// against q / 16); the 8 that a code is above its value is taken off each group's fp32 sum as 8 sum q.  q enters
-// as fp16 of q 2^-e, e the exponent of the row's largest element (exact for fp16 and bf16 inputs down to 2^-24
-// of that element); the group's scale multiplies the group's sum.  Weights: exp2 in fp32 against a running
-// reference per row.  Values: O^T = V^T (w s)^T; an 8 x 8 transpose within the warp brings the weights into
-// place.  The product of weight and V scale is rounded once to fp16 (11 bits; bf16 would lose 3 more).  The
+// against q / 16); the 8 that a code is above its value is taken off each group's fp32 sum as 8 sum q.  q enters as fp16 of
+// q 2^(12-e), e the exponent of the row's largest element (exact for fp16 inputs down to 2^-22 and for bf16 inputs down
+// to 2^-25 of that element, the dims that meet 16 nibble being 2^-4 smaller); the group's scale multiplies the
+// group's sum.  Weights: exp2 in fp32 against a running reference per row.  Values: O^T = V^T (w s)^T; an
+// 8 x 8 transpose within the warp brings the weights into place.  The product of weight and V scale is rounded once to fp16 (11 bits; bf16 would lose 3 more).  The
 // reference follows the greatest (score + exponent of the position's largest V scale), so the products stay small
 // and are rounded relative to the largest contribution, whatever the scales are.  V codes enter as nibble - 8
 // exactly (their offset, taken off a sum, would leave its rounding where a dim's large weights have code 0).  Sums of
@@ -44,6 +44,7 @@ namespace {
 
 constexpr unsigned WHOLE_TILES = 2;   // tiles of a warp up to which one CTA takes a whole item
 constexpr int NST = 2;               // ring stages of a warp
+constexpr int QUP = 12;              // log2 of what a query row's largest element is brought to
 constexpr float MOST = 32768.f;      // 2^(BELOW + RAISE): how large a product of weight and V scale may be before the reference moves
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
         }
         for (int i = 0; i < NST && c.u + i < c.u1; ++i) load(c.b, c.h, len, c.u + i);
     };
-    // Stages a segment's query rows, a row for a warp: fp16 of q 2^-e in the order of the fragments (block of 8 dims:
+    // Stages a segment's query rows, a row for a warp: fp16 of q 2^(QUP - e) in the order of the fragments (block of 8 dims:
     // pairs (0,4), (1,5) / 16, (2,6), (3,7) / 16), the groups' sums, the factor that undoes it all, the row's limit.
     auto stage_q = [&](const Segment& c) {
         const int row0 = c.rb * RB, nrows = min(RB, P.rows - row0);
@@ -213,9 +214,9 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                 big = max(big, __float_as_uint(f[i]) & 0x7fffffffu);
             }
             big = __reduce_max_sync(0xffffffffu, big);
-            const int ex = min(max((int)(big >> 23), 1), 253);
-            // 2^-(ex - 127), with the sign of the scale so that a larger sum is a larger score
-            const float down = __uint_as_float((unsigned)(254 - ex) << 23) * (P.scale_log2 < 0.f ? -1.f : 1.f);
+            const int ex = min(max((int)(big >> 23), QUP), 253);
+            // 2^(QUP - (ex - 127)), with the sign of the scale so that a larger sum is a larger score
+            const float down = __uint_as_float((unsigned)(254 - ex + QUP) << 23) * (P.scale_log2 < 0.f ? -1.f : 1.f);
             float part = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
             for (int o = 1; o < GS / V; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
             if (lane % (GS / V) == 0) s_off[r * NS + lane / (GS / V)] = part * (-8.f / 16777216.f);
             if (lane == 0) {
-                s_mul[r] = __uint_as_float((unsigned)ex << 23) * fabsf(P.scale_log2) * 16777216.f;   // 2^24: codes are subnormals
+                s_mul[r] = __uint_as_float((unsigned)ex << 23) * fabsf(P.scale_log2) * (16777216.f / (1 << QUP));   // 2^24: codes are subnormals
                 // rows that are padding see everything and are written as zeros
                 s_lim[r] = real && t < count ? max(0, len - count + t + 1) : 0x7fffffff;
             }

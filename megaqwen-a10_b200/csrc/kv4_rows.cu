@@ -12,7 +12,8 @@
 // scale brought to [2^12, 2^13) by a power of two, which keeps 7 times it within fp16: exact for the groups whose scale is
 // at least 2^-29 of the position's largest, rounded to 2^-37 of it below that (V: in single-token attention the product
 // with the weight is rounded to 2^-32 of the row's largest; K: there each group's sum is in fp32).  The powers go to the
-// scores (K) and into the weights' exponents (V).  q is fp16 of q 2^-e as in kv4_attend.cu.  Weights are exp2 in fp32
+// scores (K) and into the weights' exponents (V).  q is fp16 with the row's largest element
+// at 2^13, exact for fp16 and bf16 inputs down to 2^-27 of that element.  Weights are exp2 in fp32
 // against a reference per row, rounded to fp16 for the product (11 bits down to 2^-21 of the largest), summed in fp32
 // unrounded.  The reference moves (and O is scaled) when a weight exceeds 2^15.
 //
@@ -29,6 +30,7 @@ namespace {
 
 constexpr int ROWS = ROWS_BLOCK, TILE = 64, NTHR = 256, STAGES = 2;
 constexpr int LIFT = 12;             // log2 of what a position's largest scale is brought to: 7 * 2^(LIFT + 1) < 65504
+constexpr int QUP = 13;              // log2 of what a query row's largest element is brought to
 constexpr unsigned WHOLE_UNITS = 8;  // units up to which one CTA takes a whole item
 constexpr int TMEM_COLS = 256, O_COL = 128;
 
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
     uint8_t* s_v = s_k + G::K;
     uint8_t* s_p = s_v + G::V;
     uint8_t* raw = s_p + G::PT;
-    float* kf = reinterpret_cast<float*>(raw + STAGES * G::RAW);   // [TILE] 2^e: K is 2^e times its operand
+    float* kf = reinterpret_cast<float*>(raw + STAGES * G::RAW);   // [TILE] 2^(e - QUP): K is 2^e times its operand
     float* ve = kf + TILE;                                          // [TILE] e: V is 2^e times its operand
     float* vi = ve + TILE;                                          // [TILE] 2^-e
     __half* v16 = reinterpret_cast<__half*>(vi + TILE);             // [NS][TILE] V scales * 2^-e
@@ -260,8 +262,8 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
                 for (int o = 1; o < 8; o <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
                 big = max(big & 0xffffu, big >> 16);
                 const unsigned bits = __float_as_uint(P.dtype == MQ_BF16 ? bf16_bits_to_f32(big) : __half2float(__ushort_as_half((unsigned short)big)));
-                const int ex = min(max((int)(bits >> 23), 1), 253);
-                const float down = __uint_as_float((unsigned)(254 - ex) << 23) * (P.scale_log2 < 0.f ? -1.f : 1.f);
+                const int ex = min(max((int)(bits >> 23), QUP), 253);
+                const float down = __uint_as_float((unsigned)(254 - ex + QUP) << 23) * (P.scale_log2 < 0.f ? -1.f : 1.f);
 #pragma unroll
                 for (int c = 0; c < NCH; ++c) {
                     const uint32_t w[4] = {x[i][c].x, x[i][c].y, x[i][c].z, x[i][c].w};
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(NTHR, ROWS_CTAS) rows_kernel(const RowsParams 
                     float sc[NS];
                     unsigned nan;
                     const int ex = scales(0, p, sc, nan);
-                    if (g == 0) kf[p] = __uint_as_float((unsigned)(127 + ex) << 23);
+                    if (g == 0) kf[p] = __uint_as_float((unsigned)(127 + ex - QUP) << 23);
                     float mine = sc[0];
 #pragma unroll
                     for (int k = 1; k < NS; ++k)

@@ -65,3 +65,20 @@ def test_a_group_of_v_far_below_its_neighbours(T, D, group, down):
     q = _rand((1, T, 2, D), 3, torch.bfloat16)
     vv, smax = _held(v, group)
     _compare(c.attend(0, q, [S]), q, _held(k, group)[0], vv, smax, D ** -0.5, 2 * T > 32)
+
+
+@pytest.mark.parametrize("T", [1, 8, 50])
+@pytest.mark.parametrize("D,group", [(128, 32), (128, 64), (64, 32)])
+@pytest.mark.parametrize("down", [12, 16, 20])
+def test_a_group_of_k_far_below_its_neighbours(T, D, group, down):
+    """The queries are as much larger in that group, so its part of the scores counts as much as the others'."""
+    S = 40 + T
+    c = mq.KV4Cache(1, 1, S, num_kv_heads=1, head_dim=D, group=group)
+    k, q = _rand((1, S, 1, D), 1), _rand((1, T, 2, D), 3)
+    k[..., group:2 * group] *= 2.0 ** -down
+    q[..., group:2 * group] *= 2.0 ** down
+    k, q = k.bfloat16(), q.bfloat16()
+    v = _rand((1, S, 1, D), 2, torch.bfloat16)
+    c.append(0, k, v, [0])
+    vv, smax = _held(v, group)
+    _compare(c.attend(0, q, [S], scale=0.2), q, _held(k, group)[0], vv, smax, 0.2, 2 * T > 32)
