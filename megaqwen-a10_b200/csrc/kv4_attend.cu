@@ -13,14 +13,18 @@
 // Arithmetic.  Scores: S^T = K q^T by m16n8k16 fp16 products with fp32 sums; 16 positions are the rows of A,
 // 8 query rows the columns (an A with the queries as rows would be half empty for up to 8 of them).  A K code
 // enters as the fp16 subnormal nibble * 2^-24, which a mask alone makes (16 nibble * 2^-24 for every other one,
-// against q / 16); the 8 that a code is above its value is taken off each group's fp32 sum as 8 sum q.  q enters as fp16 of
+// against q / 16); the 8 that a code is above its value is taken off each group's fp32 sum as 8 sum q.  That leaves an
+// error of about 2^-22 of 8 max|q| s, too much where a few elements of q are far above the others (more than half of
+// them 2^-6 below the largest) and K is small in their dims.  The tiles of such a row block, and those at the end of what
+// a row sees, take the codes as signed numbers instead (32 half2 sums more for 16 positions).  q enters as fp16 of
 // q 2^(12-e), e the exponent of the row's largest element (exact for fp16 inputs down to 2^-22 and for bf16 inputs down
-// to 2^-25 of that element, the dims that meet 16 nibble being 2^-4 smaller); the group's scale multiplies the
-// group's sum.  Weights: exp2 in fp32 against a running reference per row.  Values: O^T = V^T (w s)^T; an
-// 8 x 8 transpose within the warp brings the weights into place.  The product of weight and V scale is rounded once to fp16 (11 bits; bf16 would lose 3 more).  The
-// reference follows the greatest (score + exponent of the position's largest V scale), so the products stay small
-// and are rounded relative to the largest contribution, whatever the scales are.  V codes enter as nibble - 8
-// exactly (their offset, taken off a sum, would leave its rounding where a dim's large weights have code 0).  Sums of
+// to 2^-25 of that element, the dims that meet 16 nibble being 2^-4 smaller); the group's scale multiplies the group's
+// sum.  Weights: exp2 in fp32 against a running reference per row.  Values: O^T = V^T (w s)^T; an 8 x 8 transpose within
+// the warp brings the weights into place.  The product of weight and V scale is rounded once to fp16 (11 bits; bf16 would
+// lose 3 more).  The reference follows the greatest (score + exponent of the position's largest V scale), so the products
+// stay small and are rounded relative to the largest contribution, whatever the scales are (11 bits down to 2^-21 of it,
+// 2^-32 of it below that, in the dims of a group whose scales are that far below the others' too).  V codes enter as
+// nibble - 8 exactly (their offset, taken off a sum, would leave its rounding where a dim's large weights have code 0).  Sums of
 // weights are fp32 and unrounded.  The reference moves only when a product exceeds 2^15 (a vote), so most tiles need no
 // reduction across lanes.
 //
@@ -73,6 +77,13 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Pairs of nibbles (times F, in the low bits of either half) -> fp16 pairs F (nibble - 8): the nibble in the mantissa of 1024.
+template <int F>
+__device__ __forceinline__ uint32_t signed_codes(uint32_t v) {
+    const uint32_t x = v | 0x64006400u;
+    const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(-(1024.f + 8.f * F)));
+    return *reinterpret_cast<const uint32_t*>(&y);
 }
 // Transposes an 8 x 8 matrix of 16-bit elements, row lane / 4, columns 2 (lane % 4) and + 1 in each lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -214,6 +225,10 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                 big = max(big, __float_as_uint(f[i]) & 0x7fffffffu);
             }
             big = __reduce_max_sync(0xffffffffu, big);
+            int small = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) small += fabsf(f[i]) < __uint_as_float(big) * 0x1p-6f;
+            const bool peaked = __reduce_add_sync(0xffffffffu, small) > D / 2;
             const int ex = min(max((int)(big >> 23), QUP), 253);
             // 2^(QUP - (ex - 127)), with the sign of the scale so that a larger sum is a larger score
             const float down = __uint_as_float((unsigned)(254 - ex + QUP) << 23) * (P.scale_log2 < 0.f ? -1.f : 1.f);
@@ -229,7 +244,8 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
             for (int o = 1; o < GS / V; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
             if (lane % (GS / V) == 0) s_off[r * NS + lane / (GS / V)] = part * (-8.f / 16777216.f);
             if (lane == 0) {
-                s_mul[r] = __uint_as_float((unsigned)ex << 23) * fabsf(P.scale_log2) * (16777216.f / (1 << QUP));   // 2^24: codes are subnormals
+                // 2^24: codes are subnormals; the sign says that the row's largest elements are far above the others
+                s_mul[r] = __uint_as_float((unsigned)ex << 23) * fabsf(P.scale_log2) * (16777216.f / (1 << QUP)) * (peaked ? -1.f : 1.f);
                 // rows that are padding see everything and are written as zeros
                 s_lim[r] = real && t < count ? max(0, len - count + t + 1) : 0x7fffffff;
             }
@@ -258,8 +274,9 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
         int limit[NB][2];
         uint32_t qf[NB][NG][4];
         const int lim = lane < RB ? s_lim[lane] : 0x7fffffff;
-        const int low = __reduce_min_sync(0xffffffffu, lim);                               // least and greatest limit of
+        int low = __reduce_min_sync(0xffffffffu, lim);                                     // least and greatest limit of
         const int high = __reduce_max_sync(0xffffffffu, lim == 0x7fffffff ? 0 : lim);      // the block's rows
+        if (__any_sync(0xffffffffu, lane < CR * NB && signbit(s_mul[lane]))) low = 0;      // every tile takes signed codes
         const int cg = REP ? 2 * cq / CR : 0;            // the group of this lane's columns
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -272,7 +289,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = 8 * nb + (2 * cq + i) % CR;
-                mul[nb][i] = s_mul[r];
+                mul[nb][i] = fabsf(s_mul[r]);
                 limit[nb][i] = s_lim[r];
                 ref[nb][i] = NEG_INF; sum[nb][i] = 0.f;
 #pragma unroll
@@ -286,7 +303,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                     for (int i = 0; i < 4; ++i) acc[nb][g][m][i] = 0.f;
         }
 
-        // One tile of 32 positions; EDGE: some row does not see all of it.
+        // One tile of 32 positions; EDGE: some row does not see all of it, or a row asks for signed codes.
         auto tile = [&](auto edge, const uint8_t* base, int p0) {
             constexpr bool EDGE = decltype(edge)::value;
             constexpr int SETS = REP ? 1 : NS;           // weight fragments: one, or one for each group's scales
@@ -315,8 +332,12 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const uint32_t v0 = w[0][g] >> 8, v1 = w[1][g] >> 8;
-                    const uint32_t a0 = w[0][g] & 0x000f000fu, a1 = w[1][g] & 0x000f000fu, a2 = w[0][g] & 0x00f000f0u, a3 = w[1][g] & 0x00f000f0u;
-                    const uint32_t b0 = v0 & 0x000f000fu, b1 = v1 & 0x000f000fu, b2 = v0 & 0x00f000f0u, b3 = v1 & 0x00f000f0u;
+                    uint32_t a0 = w[0][g] & 0x000f000fu, a1 = w[1][g] & 0x000f000fu, a2 = w[0][g] & 0x00f000f0u, a3 = w[1][g] & 0x00f000f0u;
+                    uint32_t b0 = v0 & 0x000f000fu, b1 = v1 & 0x000f000fu, b2 = v0 & 0x00f000f0u, b3 = v1 & 0x00f000f0u;
+                    if constexpr (EDGE) {
+                        a0 = signed_codes<1>(a0); a1 = signed_codes<1>(a1); a2 = signed_codes<16>(a2); a3 = signed_codes<16>(a3);
+                        b0 = signed_codes<1>(b0); b1 = signed_codes<1>(b1); b2 = signed_codes<16>(b2); b3 = signed_codes<16>(b3);
+                    }
                     const bool starts = REP ? g == 0 : g * 32 % GS == 0, ends = REP ? g == NG - 1 : (g + 1) * 32 % GS == 0;
                     const int gs = REP ? 0 : g * 32 / GS;
 #pragma unroll
@@ -327,7 +348,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
                         if (ends)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float z = d[nb][i] + off[nb][i & 1][gs];
+                                const float z = EDGE ? d[nb][i] * 0x1p-24f : d[nb][i] + off[nb][i & 1][gs];
                                 s[x][nb][i] = gs == 0 ? ks[i >> 1][gs] * z : fmaf(ks[i >> 1][gs], z, s[x][nb][i]);
                             }
                     }

@@ -82,3 +82,19 @@ def test_a_group_of_k_far_below_its_neighbours(T, D, group, down):
     c.append(0, k, v, [0])
     vv, smax = _held(v, group)
     _compare(c.attend(0, q, [S], scale=0.2), q, _held(k, group)[0], vv, smax, 0.2, 2 * T > 32)
+
+
+@pytest.mark.parametrize("T", [1, 8, 50])
+@pytest.mark.parametrize("dtype,up", [(torch.bfloat16, 5), (torch.float16, 7), (torch.bfloat16, 9), (torch.bfloat16, 16), (torch.bfloat16, 20),
+                                      (torch.float16, 12), (torch.float16, 14)])
+def test_a_large_element_of_the_query(T, dtype, up):
+    """One dim of the queries far above the others, where K is zero: the scores are the others' alone."""
+    S, D = 40 + T, 128
+    c = mq.KV4Cache(1, 1, S, num_kv_heads=1)
+    k, q = _rand((1, S, 1, D), 1), _rand((1, T, 2, D), 3)
+    k[..., 40] = 0.0
+    q[..., 40] = 2.0 ** up
+    k, q, v = k.bfloat16(), q.to(dtype), _rand((1, S, 1, D), 2, torch.bfloat16)
+    c.append(0, k, v, [0])
+    vv, smax = _held(v, 32)
+    _compare(c.attend(0, q, [S], scale=0.2), q, _held(k, 32)[0], vv, smax, 0.2, 2 * T > 32)
