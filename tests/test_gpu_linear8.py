@@ -254,3 +254,15 @@ def test_captured_calls_keep_their_workspace():
         graph.replay()                 # on the current stream, while `side` may still run
     torch.cuda.synchronize()
     assert torch.equal(y, want) and all(torch.equal(b, want_big) for b in beside)
+
+
+# M * K = 8192 codes are the most that the kernel for few tokens takes; one 16-byte unit more goes to the tensor cores
+@pytest.mark.parametrize("m,k", [(1, 8192), (2, 4096), (4, 2048), (1, 8208), (4, 2064)])
+def test_largest_sums_of_few_tokens(m, k):
+    """All codes at their extremes, on both sides of the rule between the kernels; signs that alternate in the second row."""
+    s = torch.ones(16, device="cuda")
+    for value in (-128, 127):
+        w = torch.full((16, k), value, dtype=torch.int8, device="cuda")
+        x = torch.ones((m, k), device="cuda")
+        x[m - 1, 1::2] = -1.0 if m > 1 else 1.0
+        check(mq.Int8Linear(w, s)(x), reference(x, w, s))
