@@ -412,7 +412,15 @@ int mq_kv4_read(const MQKV4Cache* cache, const int* starts, int n, int dtype, vo
  *   - lengths: device int32 [batch], positions held, the new tokens included;
  *     counts: device int32 [batch] or NULL (all `tokens`): row t of sequence b is
  *     at position lengths[b] - counts[b] + t and sees positions 0 .. its own; a
- *     row with t >= counts[b], or before position 0, gives zeros.
+ *     row with t >= counts[b], or before position 0, gives zeros.  Where counts[b]
+ *     is 0 nothing of sequence b is needed, and its page table entries may hold
+ *     anything.
+ *   - precision: scores, sums and the softmax statistics are fp32; q enters
+ *     exactly down to 2^-22 of its row's largest element; weights times V scales (up
+ *     to 32 query rows of a KV head) or weights (more) are rounded to fp16, 11 bits
+ *     down to 2^-21 of the row's largest and 2^-32 of it below; for more than 32
+ *     rows, a scale more than 2^29 below its position's largest is rounded to
+ *     2^-37 of that.
  *   - workspace (scratch) and counters (int32, zero before the first use, left
  *     zero): as large as mq_kv4_attend_workspace says; calls on different
  *     streams need their own, host threads on one stream may share them.
@@ -427,6 +435,7 @@ int mq_kv4_attend(const MQKV4Cache* cache, int dtype, const void* q, const int64
  * Linear product in 8-bit integers (the reference's INT8 path keeps activations
  * in floating point): y[m][n] = (sum_k c[m][k] w[n][k]) * s_x[m] * w_scale[n], where
  * s_x[m] = max(fp32(max_k |x[m][k]| / 127), 1e-12) and c = round half even (x / s_x).
+ * The two scales are multiplied first, in fp32, whose range their product must keep.
  *   - x: [M][K] of `dtype`, row stride x_stride elements, contiguous rows;
  *     w: int8 [N][K], row stride w_stride bytes: a multiple of 16 and at least K
  *     rounded up to 16, whose bytes up to there are readable (their values do not

@@ -35,10 +35,10 @@
 // A segment's fixed costs are latency, and much of that is fetching instructions that run once, so the code around
 // the tiles is written small: queries go through shared memory, joins take one output each.
 //
-// Measured, 16 heads over 8 of 128 dims, group 32: 64 sequences of 128 to 4096 (156 MB of codes and scales) 51 us,
-// 3.1 TB/s -- 2.1 us of it the whole cache's products, the rest instructions (53 % of the issue slots; half of them run
-// at half rate), about 6 us before the first tile and the spread of the CTAs' ends; one sequence of 32768 21 us, of which
-// 7 are tiles; one of 200 6 us, which is latency.
+// Measured, 16 heads over 8 of 128 dims, group 32: 64 sequences of 128 to 4096 (156 MB of codes and scales) 52 us,
+// 3.0 TB/s -- 2.1 us of it the whole cache's products, the rest instructions (53 % of the issue slots; half of them run
+// at half rate), about 6 us before the first tile and the spread of the CTAs' ends; one sequence of 32768 22 us, of which
+// 7 are tiles; one of 200 7 us, which is latency.  Queries that ask for signed codes: 64 sequences 65 us.
 #include <type_traits>
 #include "kv4_plan.cuh"
 
@@ -695,6 +695,7 @@ int g_sm_count[MAX_DEV];
 //   4 sequences of 6000                   29.5  46.6   40.8  47.1   51.0  47.9   60.8  48.1
 //   32 sequences of 128 to 4096                        115   118    173   119    228   120
 //   1 sequence of 3000                                 21.9  23.6   18.1  24.1   23.7  24.1
+// The rule looks at the rows alone: one short sequence with 33 to 64 rows would be up to 6 us quicker in blocks of 16.
 int block_rows(int rows) { return rows <= 8 ? 8 : rows <= 32 ? 16 : ROWS_BLOCK; }
 
 int sm_count(int& n) {

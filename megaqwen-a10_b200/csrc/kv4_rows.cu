@@ -17,9 +17,9 @@
 // against a reference per row, rounded to fp16 for the product (11 bits down to 2^-21 of the largest), summed in fp32
 // unrounded.  The reference moves (and O is scaled) when a weight exceeds 2^15.
 //
-// Measured: 4 sequences of 1000 to 6001 positions, 64 tokens each, 16 heads over 8 of 128 dims: 39.5 us with the joins
-// (88 TFLOP/s; the products alone would take 2 us).  A tile takes a CTA 3.2 us, most of it turning codes into operands and
-// scores into weights (49 % of the issue slots with two CTAs on an SM) between barriers; the queries 4 us at the start,
+// Measured: 4 sequences of 1000 to 6001 positions, 64 tokens each, 16 heads over 8 of 128 dims: 40 us with the joins
+// (87 TFLOP/s; the products alone would take 2 us).  A tile takes a CTA 3.2 us, most of it turning codes into operands and
+// scores into weights (46 % of the issue slots with two CTAs on an SM) between barriers; the queries 4 us at the start,
 // the joins 5 at the end.
 #include "kv4_plan.cuh"
 #include "launch_lock.h"

@@ -17,9 +17,10 @@
 //     channels and the columns 16 to 256 tokens, so that few tokens waste no tensor work.
 //   * Where the tiles are too few for the SMs, a cluster of 2, 4 or 8 CTAs shares a tile along K; the partial sums
 //     meet through distributed shared memory, in integers, so the result does not depend on the split.
-// Measured with the quantiser: 64 tokens x 151936 channels x K 1024 to fp32 (195 MB) 35 us, 5.6 TB/s, bound by the
-// memory; 37 x 1024 x 3072 7.8 us, two launches' latency and 24 slabs over 8 CTAs; 8192 x 6144 x 1024 56 us (1.8
-// Pop/s), bound by bringing operands into the SMs (gemm_pair_kernel).
+// Measured with the quantiser: 64 tokens x 151936 channels x K 1024 to fp32 (195 MB) 35.6 us, 5.5 TB/s, bound by the
+// memory; 37 x 1024 x 3072 8.2 us, two launches' latency and 24 slabs over 8 CTAs; 8192 x 6144 x 1024 57 us (1.8
+// Pop/s), of which 43 us are slabs (0.48 us for 32 KB of operands in each SM, 2.4 Pop/s, also at larger K) and the rest the
+// quantiser and the tiles' ends (gemm_pair_kernel).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -684,8 +685,7 @@ __global__ void __launch_bounds__(Gemm<BN>::THREADS, 1) gemm_kernel(const __grid
 // ------------------------------------------------------------------ pairs of CTAs
 // Two CTAs of a cluster share a tile of 256 tokens x 256 channels (tcgen05.mma cta_group::2, M = 256): each brings
 // its own 128 tokens of x and half of the channels of W, and has its tokens' sums in its own TMEM.  The operands of
-// a tile cross from L2 once for both: 32 KB a slab and CTA instead of 48, which is what bounds the single-CTA tile
-// (8192 tokens x 6144 channels x K 1024, with the quantiser: 61 -> 58 us).
+// a tile cross from L2 once for both: 32 KB a slab and CTA instead of 48 (8192 tokens x 6144 channels x K 1024, with the quantiser: 61 -> 58 us).
 __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
