@@ -210,8 +210,9 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
         constexpr int V = D / 32;     // dims of a lane
 #pragma unroll 1
         for (int r = warp; r < (REP ? CR : RB); r += NW) {
-            const bool real = r < nrows;
-            const int t = real ? (row0 + r) / P.share : 0, j = real ? row0 + r - t * P.share : 0;
+            const int t = r < nrows ? (row0 + r) / P.share : 0;
+            const bool real = r < nrows && t < count;          // else no row, or padding: zeros that nothing depends on
+            const int j = real ? row0 + r - t * P.share : 0;
             const uint16_t* src = reinterpret_cast<const uint16_t*>(P.q) + (long long)c.b * P.qb + (long long)t * P.qt +
                                   (long long)(c.h * P.share + j) * P.qh + V * lane;
             uint16_t raw[V];
@@ -246,8 +247,7 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
             if (lane == 0) {
                 // 2^24: codes are subnormals; the sign says that the row's largest elements are far above the others
                 s_mul[r] = __uint_as_float((unsigned)ex << 23) * fabsf(P.scale_log2) * (16777216.f / (1 << QUP)) * (peaked ? -1.f : 1.f);
-                // rows that are padding see everything and are written as zeros
-                s_lim[r] = real && t < count ? max(0, len - count + t + 1) : 0x7fffffff;
+                s_lim[r] = real ? max(0, len - count + t + 1) : 0x7fffffff;   // else: as the row that sees most (below)
             }
         }
     };
@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(NW * 32, NW > 4 ? 1 : NB == 1 ? 4 : 2) attend_
             for (int i = 0; i < 2; ++i) {
                 const int r = 8 * nb + (2 * cq + i) % CR;
                 mul[nb][i] = fabsf(s_mul[r]);
-                limit[nb][i] = s_lim[r];
+                limit[nb][i] = min(s_lim[r], high);   // a row without a token must not weigh what was never loaded: its
+                                                      // votes move the references of the others
                 ref[nb][i] = NEG_INF; sum[nb][i] = 0.f;
 #pragma unroll
                 for (int gs = 0; gs < (REP ? 1 : NS); ++gs) off[nb][i][gs] = s_off[r * NS + (REP ? cg : gs)];
