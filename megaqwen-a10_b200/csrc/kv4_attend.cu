@@ -37,7 +37,7 @@
 //
 // Measured, 16 heads over 8 of 128 dims, group 32: 64 sequences of 128 to 4096 (156 MB of codes and scales) 52 us,
 // 3.0 TB/s -- 2.1 us of it the whole cache's products, the rest instructions (53 % of the issue slots; half of them run
-// at half rate), about 6 us before the first tile and the spread of the CTAs' ends; one sequence of 32768 22 us, of which
+// at half rate), about 6 us before the first tile and the spread of the CTAs' ends; one sequence of 32768 22.5 us, of which
 // 7 are tiles; one of 200 7 us, which is latency.  Queries that ask for signed codes: 64 sequences 65 us.
 #include <type_traits>
 #include "kv4_plan.cuh"
